@@ -237,14 +237,9 @@ def _prepare_attn(case, gen):
 
 
 # ---- one pass ---------------------------------------------------------------
-_OPS = []
-
-
 def _ops():
-    if not _OPS:  # imported once, as a program's import statement does
-        import importlib
-        _OPS.append(importlib.import_module("gemma4-12b-snapdragonx2elite_amd.ops"))
-    return _OPS[0]
+    import importlib
+    return importlib.import_module("gemma4-12b-snapdragonx2elite_amd.ops")
 
 
 def run(state):
