@@ -156,8 +156,9 @@ constexpr int PG_FEW_ROWS = 64;
 constexpr float PG_LOG2E = 1.4426950408889634f;
 // A row's weights are 2^(score - ref): ref is set 6 below the row's largest
 // score so far (in log2 units) and moves only when a score passes it by 14,
-// so weights reach 2^14 < 65504 and those 2^20 below the largest keep fp16's
-// full precision; moving it rescales the accumulators, which is rare.
+// so weights reach 2^14 < 65504 and the leading bits of those 2^20 below the
+// largest are no fp16 subnormals; moving it rescales the accumulators, which
+// is rare.
 constexpr float PG_BELOW = 6.0f, PG_MOVE = 14.0f;
 
 template <int HD>
@@ -191,6 +192,8 @@ __device__ inline void lds_write(uint32_t at, T v) {
 }
 typedef __fp16 v4hp __attribute__((ext_vector_type(4)));
 typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+// two values rounded towards zero to fp16
+__device__ inline v2h cvt_rtz(float a, float b) { return __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(a, b)); }
 __device__ inline v8h join(v4h a, v4h b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 // 4 fp16 of 16 consecutive row elements each, 4 rows per 16 lanes; the lane
 // gets the element of its number from each of the 4 rows
@@ -355,13 +358,18 @@ __device__ __forceinline__ void pg_scores(const PgLane<HD>& at, const v8h (&qf)[
 
 // Weights of a lane's scores (NST subtiles of 4 keys; -inf where masked) as
 // 2^(s log2e - ref), and the move of ref. acc: NA accumulators to rescale;
-// sum: of the lane's keys, before their rounding to fp16 (whose errors are
-// random and cancel in a sum; a product with ones for V would sum the rounded
-// weights in the matrix cores, but takes 4 registers a row instead of one).
+// sum: of the lane's keys in fp32. A weight is the sum of two fp16 values, its
+// leading bits and what they leave over, to 2^-20 of itself (rounded towards
+// zero: two at a time in one instruction; 2^-30 of the row's largest where the
+// second one is subnormal): the output is the mean of V rows under the weights
+// that the sum holds, also where one key has nearly all of the weight.
 // HL: lanes 8 .. 15 of a row's 16 hold the same rows as lanes 0 .. 7 and take
-// the part of the weight that fp16 leaves over.
+// the second values (w[0] of such a lane); else a lane has both.
+template <bool HL>
+constexpr int PG_PARTS = HL ? 1 : 2;
 template <int NST, int NA, bool HL>
-__device__ __forceinline__ void pg_weights(const v4f (&s)[NST], float& ref, v4f (&acc)[NA], float& sum, v4h (&w)[NST]) {
+__device__ __forceinline__ void pg_weights(const v4f (&s)[NST], float& ref, v4f (&acc)[NA], float& sum,
+                                           v4h (&w)[PG_PARTS<HL>][NST]) {
   float top = -INFINITY;
 #pragma unroll
   for (int st = 0; st < NST; ++st)
@@ -383,32 +391,47 @@ __device__ __forceinline__ void pg_weights(const v4f (&s)[NST], float& ref, v4f 
 #pragma unroll
   for (int st = 0; st < NST; ++st)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float p = __builtin_amdgcn_exp2f(fmaf(s[st][e], PG_LOG2E, -r));
-      sum += p;
-      const _Float16 hi = (_Float16)p;
-      if constexpr (HL) w[st][e] = (threadIdx.x & 8) ? (_Float16)(p - (float)hi) : hi;
-      else w[st][e] = hi;
+    for (int e = 0; e < 4; e += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[st][e], PG_LOG2E, -r));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(s[st][e + 1], PG_LOG2E, -r));
+      sum += p0;
+      sum += p1;
+      const v2h hi = cvt_rtz(p0, p1);
+      const v2h lo = cvt_rtz(fmaf((float)hi[0], -1.0f, p0), fmaf((float)hi[1], -1.0f, p1));
+      if constexpr (HL) {
+        const bool low = threadIdx.x & 8;
+        w[0][st][e] = low ? lo[0] : hi[0];
+        w[0][st][e + 1] = low ? lo[1] : hi[1];
+      } else {
+        w[0][st][e] = hi[0], w[0][st][e + 1] = hi[1];
+        w[1][st][e] = lo[0], w[1][st][e + 1] = lo[1];
+      }
     }
 }
 
-// O^T += V^T P^T
-template <int HD, int NST, int NR, int NDT, int DEPTH>
-__device__ __forceinline__ void pg_values(const PgLane<HD>& at, const v4h (&w)[NR][NST], v4f (&acc)[NR][NDT]) {
-  if constexpr (NST == 1) {
+// O^T += V^T P^T, for both parts of the weights
+template <int HD, int NST, int NR, int NDT, int DEPTH, int PARTS>
+__device__ __forceinline__ void pg_values(const PgLane<HD>& at, const v4h (&w)[NR][PARTS][NST], v4f (&acc)[NR][NDT]) {
+  if constexpr (NST == 1) {  // both parts in one MFMA of 32 products, as 16 keys twice: the time of one of 16
     read_ahead<NDT, DEPTH, v4h>([&](auto i) { return at.template v<0, i.value>(); },
                                 [&](auto i, v4h v) {
 #pragma unroll
                                   for (int r = 0; r < NR; ++r)
-                                    acc[r][i.value] = __builtin_amdgcn_mfma_f32_16x16x16f16(v, w[r][0], acc[r][i.value], 0, 0, 0);
+                                    if constexpr (PARTS == 2)
+                                      acc[r][i.value] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                          join(v, v), join(w[r][0][0], w[r][1][0]), acc[r][i.value], 0, 0, 0);
+                                    else
+                                      acc[r][i.value] = __builtin_amdgcn_mfma_f32_16x16x16f16(v, w[r][0][0], acc[r][i.value], 0, 0, 0);
                                 });
   } else {
     constexpr int NP = NST / 2;  // pairs of subtiles: 32 keys of one MFMA
-    v8h wp[NR][NP];
+    v8h wp[NR][PARTS][NP];
 #pragma unroll
     for (int r = 0; r < NR; ++r)
 #pragma unroll
-      for (int k = 0; k < NP; ++k) wp[r][k] = join(w[r][2 * k], w[r][2 * k + 1]);
+      for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+        for (int k = 0; k < NP; ++k) wp[r][p][k] = join(w[r][p][2 * k], w[r][p][2 * k + 1]);
     read_ahead<NDT * NP, DEPTH, v8h>(
         [&](auto i) {
           constexpr int d = i.value / NP, k = i.value % NP;
@@ -417,7 +440,10 @@ __device__ __forceinline__ void pg_values(const PgLane<HD>& at, const v4h (&w)[N
         [&](auto i, v8h v) {
           constexpr int d = i.value / NP, k = i.value % NP;
 #pragma unroll
-          for (int r = 0; r < NR; ++r) acc[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, wp[r][k], acc[r][d], 0, 0, 0);
+          for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+              acc[r][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, wp[r][p][k], acc[r][d], 0, 0, 0);
         });
   }
 }
@@ -511,7 +537,8 @@ __device__ __forceinline__ void shared_role(const PgArgs& a, const Pages& pg, ui
   using S = PgTile<HD>;
   constexpr int KT = S::KT, NST = KT / 16, DS = S::DS, NCH = S::NCH / DS, NDT = S::NDT / DS;
   constexpr int NW = PG_WAVES * DS, KW = KT / NW, HW = HD / DS;
-  constexpr int DEPTH = DS == 2 ? 3 : 4;  // (a fourth spills)
+  constexpr int DEPTH = DS == 2 ? 3 : 4;  // (a fourth spills in the tile loop; with three, one
+                                          // register is saved before it and read back behind it)
   const int kvh = bid % a.nkv, split = bid / a.nkv % a.nsp, rb = bid / (a.nkv * a.nsp);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15,
             g = lane >> 4, dp = wave % DS;
@@ -610,10 +637,10 @@ __device__ __forceinline__ void shared_role(const PgArgs& a, const Pages& pg, ui
               if (!(held(id[st]) && key < k1 && rows.has(r, key, a.window))) s[r][st][e] = -INFINITY;
             }
       }
-      v4h w[NR][NST];
+      v4h w[NR][2][NST];
 #pragma unroll
       for (int r = 0; r < NR; ++r) pg_weights<NST, NDT, false>(s[r], ref[r], acc[r], sum[r], w[r]);
-      pg_values<HD, NST, NR, NDT, 4>(at, w, acc);
+      pg_values<HD, NST, NR, NDT, DEPTH>(at, w, acc);
     }
     at.move(by);
 #pragma unroll
@@ -730,7 +757,7 @@ __device__ __forceinline__ void stream_role(const PgArgs& a, const Pages& pg, ui
           if (!(held(id[st]) && key < k1 && in)) s[0][st][e] = -INFINITY;
         }
     }
-    v4h w[1][NST];
+    v4h w[1][PG_PARTS<HL>][NST];
     pg_weights<NST, NDT, HL>(s[0], ref, acc[0], sum, w[0]);
     if (more) vmwait<NI>();
     else vmwait<0>();
@@ -792,8 +819,8 @@ __device__ __forceinline__ void stream_role(const PgArgs& a, const Pages& pg, ui
   }
 }
 
-// HL: up to 8 query heads per KV head, so the own pages' weights keep their
-// low parts.
+// HL: up to 8 query heads per KV head, so that the idle lanes of the own
+// pages' rows take the weights' second parts.
 template <int HD, int MODE, bool HL>
 __global__ void __launch_bounds__(PgTile<HD>::threads(MODE), PgTile<HD>::waves(MODE))
 paged_attn_kernel(const PgArgs a, const Pages pg) {
@@ -1036,7 +1063,7 @@ int q4_paged_attn(const uint16_t* q, int ldq, const uint16_t* kc, const uint16_t
   const long grid = (long)p.nrb * nkv * p.nsp + (long)T * nkv * p.nhb * p.nso;
   Q4_ARG(grid < PG_MAX_BLOCKS / 2 && (long)T * nH < PG_MAX_BLOCKS, "a batch of %d rows of %d heads is too large", T, nH);
   hipStream_t st = as_stream(stream);
-  const bool hl = nH / nkv <= 8;  // a group's heads leave room in 16 rows for their weights' low parts
+  const bool hl = nH / nkv <= 8;  // a group's heads leave room in 16 rows for their weights' second parts
 #define PG_LAUNCH(HD, MODE) \
   const dim3 threads(PgTile<HD>::threads(MODE));                                                                   \
   if (hl) hipLaunchKernelGGL((paged_attn_kernel<HD, MODE, true>), dim3((unsigned)grid), threads, 0, st, a, pg); \

@@ -595,7 +595,8 @@ int q4_paged_prep(const void* qkv, int dtype, int ld, int qoff, int koff, int vo
  * zeros. Cache rows must be finite from the first to the last key attended
  * there, by its row in own pages, by any row in the prefix (without a
  * window: the whole prefix); all others may hold anything. Softmax
- * statistics and sums in fp32; the weights enter the V product as fp16. ws:
+ * statistics and sums in fp32; a weight enters the V product as the sum of two
+ * fp16 values, to 2^-20 of itself. ws:
  * q4_paged_attn_workspace_bytes bytes, 16-byte aligned, no initialisation,
  * one per stream (0: none needed, may be NULL). q, kc, vc, out 16-byte
  * aligned, ldq and ldo multiples of 8; out and ws may not overlap each other,

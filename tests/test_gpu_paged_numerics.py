@@ -1,0 +1,61 @@
+"""Precision of paged attention (paged_attn), in each of its forms: own pages
+with up to 8 query heads per KV head and with more, and a prefix with few,
+some and many query rows per KV head.
+
+Tolerances. A softmax weight is held as two fp16 values, to 2^-20 of itself;
+the score and its exponential are off by 1e-5 relative of the weight for
+|score differences| up to 30; a wave adds n keys' products, and as many
+weights, in fp32: n * 2^-24 at most. So the quotient of the two sums is off by
+2 (1e-5 + 2^-20 + n 2^-24) max|V| at most, with n up to 128 here 4e-5 max|V|,
+before its rounding to fp16, half a step: 2^-11 of the value (2^-25 in the
+subnormals).
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged_oracle as G
+from test_gpu_paged import F16, _attn_case, _np, _run_attn
+
+pytestmark = pytest.mark.gpu
+
+# form: (query heads, KV heads, prefix, own keys of each row)
+FORMS = {"own": (8, 4, 0, [1, 5, 40, 200, 33, 64]),
+         "own_wide": (20, 1, 0, [1, 5, 40, 200, 33, 64]),
+         "prefix_stream": (8, 4, 300, [1, 2, 5]),
+         "prefix_64_rows": (16, 2, 300, [1, 2, 5, 30, 7]),
+         "prefix_128_rows": (16, 2, 300, [1 + i for i in range(12)])}
+
+
+def _case(form, hd, seed, **kw):
+    nH, nkv, P, lens = FORMS[form]
+    return _attn_case(seed + hd, nH, nkv, hd, 32, P, lens, 0, 0, **kw)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("form", FORMS)
+def test_equal_values_come_out_unchanged(gpu, form, hd):
+    """The output is a mean of V rows under weights that sum to one: where all
+    keys have one V row it is that row, whatever the weights, since less than
+    2^-12 relative is lost before the rounding to fp16. Scores of a spread
+    that leaves most of a row's weight to a few keys."""
+    c = _case(form, hd, 40, spread=4.0, poison=False)
+    nkv = c["kc"].shape[1]
+    v = np.random.default_rng(hd).standard_normal((nkv, hd)).astype(np.float16)
+    c["vc"][:] = v[None, :, None, :]
+    got = _np(_run_attn(gpu, c)).reshape(len(c["q"]), nkv, c["nH"] // nkv, hd)
+    off = got != v[None, :, None, :]
+    assert not off.any(), f"{int(off.sum())} of {off.size} values off"
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("spread", [1.5, 4.0])
+def test_weights_keep_their_low_bits(gpu, form, hd, spread):
+    c = _case(form, hd, 50, spread=spread)
+    got = _np(_run_attn(gpu, c)).astype(np.float64)
+    ref = np.stack(G.paged_attn_ref(c["q"], c["kc"], c["vc"], nH=c["nH"], table=c["table"], seq=c["seq"], pos=c["pos"],
+                                    P=c["P"], prefix_pages=c["pre"]))
+    vmax = float(np.abs(c["vc"][np.isfinite(c["vc"])]).max())
+    off = np.abs(got - ref) - (np.abs(ref) * 2.0 ** -11 + 2.0 ** -25 + 4e-5 * vmax)
+    assert (off <= 0).all(), (int((off > 0).sum()), off.max())
