@@ -692,6 +692,7 @@ __device__ __forceinline__ void stream_role(const PgArgs& a, const Pages& pg, ui
     if (!pg_token<true>(pg, t, a.window, P, s, lo, hi)) return;  // (uniform) no row
     lo = max(0, lo - P);
     hi -= P;
+    if (hi <= lo) lo = hi = 0;  // no keys (a position far past max_own: lo + split * per would pass 32 bits)
     tab = pg.table + (long)s * pg.ld;
     wlo = lo, whi = hi;
   } else {

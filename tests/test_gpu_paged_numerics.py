@@ -59,3 +59,21 @@ def test_weights_keep_their_low_bits(gpu, form, hd, spread):
     vmax = float(np.abs(c["vc"][np.isfinite(c["vc"])]).max())
     off = np.abs(got - ref) - (np.abs(ref) * 2.0 ** -11 + 2.0 ** -25 + 4e-5 * vmax)
     assert (off <= 0).all(), (int((off > 0).sum()), off.max())
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("P", [0, 200])
+def test_positions_far_past_the_own_keys(gpu, hd, P):
+    """Windows that begin up to 2^31 - 1, in every split of the own keys: such
+    a row has no keys and gives zeros; its neighbours keep theirs."""
+    c = _attn_case(hd + P, 8, 4, hd, 16, P, [700, 3, 64, 1, 1, 1], 0, 0, poison=False)
+    for window in (1, 64, 1024):
+        c.update(window=window, pos=[P + 699, 2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 1500, P, 2 ** 31 - 30000])
+        got = _np(_run_attn(gpu, c)).astype(np.float64)
+        max_own = 16 * c["table"].shape[1]
+        assert not got[[1, 2, 3, 5]].any()
+        ref = G.paged_attn_ref(c["q"], c["kc"], c["vc"], nH=8, table=c["table"], seq=c["seq"], pos=c["pos"], P=P,
+                               prefix_pages=c["pre"], window=window, max_own=max_own)
+        for t in (0, 4):
+            off = np.abs(got[t] - ref[t]) - (np.abs(ref[t]) * 2.0 ** -11 + 2.0 ** -25 + 4e-5 * np.abs(c["vc"]).max())
+            assert (off <= 0).all(), (t, window, off.max())
