@@ -317,11 +317,15 @@ __device__ inline void load_q(const uint16_t* q, int g, v8h (&qf)[N]) {
 // Its registers, zeros where there is no row. The compiler's wait for the
 // loads stands here, behind the first tile's loads and before the tile loop,
 // where it would wait for that loop's loads.
+// An Inf becomes a NaN (q 0 + q, which leaves all finite values): the softmax
+// over scores that hold one is NaN in either case, and so that all of them are
+// NaN, not -inf as where a key is masked.
 template <int N>
 __device__ inline void settle(v8h (&qf)[N], bool live) {
+  const v8h zero = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    if (!live) qf[j] = v8h{0, 0, 0, 0, 0, 0, 0, 0};
+    qf[j] = live ? __builtin_elementwise_fma(qf[j], zero, qf[j]) : zero;
     pin(qf[j]);
   }
 }
@@ -357,12 +361,13 @@ __device__ __forceinline__ void pg_scores(const PgLane<HD>& at, const v8h (&qf)[
 }
 
 // Weights of a lane's scores (NST subtiles of 4 keys; -inf where masked) as
-// 2^(s log2e - ref), and the move of ref. acc: NA accumulators to rescale;
-// sum: of the lane's keys in fp32. A weight is the sum of two fp16 values, its
-// leading bits and what they leave over, to 2^-20 of itself (rounded towards
-// zero: two at a time in one instruction; 2^-30 of the row's largest where the
-// second one is subnormal): the output is the mean of V rows under the weights
-// that the sum holds, also where one key has nearly all of the weight.
+// 2^(s log2e - ref), and the move of ref. A NaN passes the maximum by and ends
+// in sum and acc. acc: NA accumulators to rescale; sum: of the lane's keys in
+// fp32. A weight is the sum of two fp16 values, its leading bits and what they
+// leave over, to 2^-20 of itself (rounded towards zero: two at a time in one
+// instruction; 2^-30 of the row's largest where the second one is subnormal):
+// the output is the mean of V rows under the weights that the sum holds, also
+// where one key has nearly all of the weight.
 // HL: lanes 8 .. 15 of a row's 16 hold the same rows as lanes 0 .. 7 and take
 // the second values (w[0] of such a lane); else a lane has both.
 template <bool HL>
@@ -408,6 +413,11 @@ __device__ __forceinline__ void pg_weights(const v4f (&s)[NST], float& ref, v4f 
       }
     }
 }
+
+// The reference that a row's part leaves, -inf where it has no keys. Where
+// its sum is NaN +inf, so that the join takes it for the largest: the other
+// parts' factors are then 0, this one's 2^(inf - inf) and the output are NaN.
+__device__ inline float part_ref(float ref, float sum) { return sum == sum ? ref : INFINITY; }
 
 // O^T += V^T P^T, for both parts of the weights
 template <int HD, int NST, int NR, int NDT, int DEPTH, int PARTS>
@@ -653,6 +663,7 @@ __device__ __forceinline__ void shared_role(const PgArgs& a, const Pages& pg, ui
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
     const float l = slot_reduce<16>(sum[r]);
+    ref[r] = part_ref(ref[r], l);
     if (rows.pos[r] < 0) continue;
     const long part = pg_part(a, rows.row(a, kvh, r0 + 16 * r + c), split);
     if (g == 0 && dp == 0) {
@@ -776,7 +787,7 @@ __device__ __forceinline__ void stream_role(const PgArgs& a, const Pages& pg, ui
   for (int d = 0; d < NDT; ++d) lds_write<v4f>(kt + c * HD * 4 + 16 * ((4 * d + g) ^ c), acc[0][d]);
   const float l = slot_reduce<16>(sum);
   if (g == 0) {
-    ml[wave][c][0] = ref;
+    ml[wave][c][0] = part_ref(ref, l);
     ml[wave][c][1] = l;
   }
   __syncthreads();

@@ -77,3 +77,40 @@ def test_positions_far_past_the_own_keys(gpu, hd, P):
         for t in (0, 4):
             off = np.abs(got[t] - ref[t]) - (np.abs(ref[t]) * 2.0 ** -11 + 2.0 ** -25 + 4e-5 * np.abs(c["vc"]).max())
             assert (off <= 0).all(), (t, window, off.max())
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("form", [*FORMS, "own_one_part"])
+def test_nonfinite_queries_give_nan(gpu, form, hd):
+    """A query head with a NaN or an Inf has no finite score, so that its
+    softmax is NaN in fp32 arithmetic, however the keys are split; all others
+    keep their bits. An Inf times negative keys alone (all scores -inf) and one
+    times a 0 (a NaN score) are among them."""
+    if form == "own_one_part":
+        c = _attn_case(60 + hd, 8, 4, hd, 32, 0, [1, 5, 30, 64], 0, 0, poison=False)
+        assert gpu.paged_attn_workspace(4, 8, 4, hd, 0, 64) is None
+    else:
+        c = _case(form, hd, 60, poison=False)
+    c["kc"][..., 1] = -np.abs(c["kc"][..., 1]) - 1
+    c["kc"][..., 2] = 0
+    want = _np(_run_attn(gpu, c)).copy()
+    T, nH = len(c["q"]), c["nH"]
+    hit = np.zeros((T, nH, hd), bool)
+    q = c["q"].reshape(T, nH, hd)
+    for i, (e, x) in enumerate([(0, np.nan), (hd - 1, np.inf), (hd // 2 + 3, -np.inf), (1, np.inf), (1, -np.inf), (2, np.inf),
+                                (hd // 2 + 9, np.nan)]):
+        t, h = i * 5 % T, (3 * i + 1) % nH
+        q[t, h, e] = x
+        hit[t, h] = True
+    got = _np(_run_attn(gpu, c))
+    hit = hit.reshape(T, -1)
+    assert np.isnan(got[hit]).all()
+    assert (got[~hit] == want[~hit]).all()
+
+
+def test_nonfinite_queries_without_keys_give_zeros(gpu):
+    c = _attn_case(71, 16, 8, 256, 16, 40, [40, 20, 5], 0, 0, poison=False)
+    c["table"][1, :] = -1
+    c["pre"][:] = -1
+    c["q"][1, 3], c["q"][1, 300] = np.nan, np.inf
+    assert not _np(_run_attn(gpu, c))[1].any()
