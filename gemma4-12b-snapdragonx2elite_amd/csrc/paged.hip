@@ -27,7 +27,9 @@ struct Pages {
   const int32_t* seq;           // [T]: sequence of each row, out of range = no row
   const int32_t* pos;           // [T]: its position
   int ld, nseq, npages, lg, max_prefix, max_own;
-  __device__ inline int prefix() const { return prefix_len ? min(max(uload(prefix_len, 0), 0), max_prefix) : 0; }
+  // P, which divides the positions; attention visits its first max_prefix keys
+  __device__ inline int prefix() const { return prefix_len ? max(uload(prefix_len, 0), 0) : 0; }
+  __device__ inline int prefix_keys() const { return min(prefix(), max_prefix); }
 };
 
 // ---- q, k, v rows: norm, RoPE, append ---------------------------------------
@@ -470,13 +472,12 @@ __device__ inline long pg_part(const PgArgs& a, int row, int part) { return (lon
 template <int HD>
 __device__ inline float* pg_ml(const PgArgs& a, long part) { return a.ws + (long)a.T * a.nH * a.np * HD + 2 * part; }
 
-// Token t's sequence, first key, and the key after its last (prefix + own, absolute).
+// Token t's sequence, position and the first position that it attends.
 template <bool UNIFORM>
-__device__ inline bool pg_token(const Pages& pg, int t, int window, int P, int& s, int& lo, int& hi) {
+__device__ inline bool pg_token(const Pages& pg, int t, int window, int& s, int& pos, int& lo) {
   s = UNIFORM ? uload(pg.seq, t) : pg.seq[t];
-  const int pos = UNIFORM ? uload(pg.pos, t) : pg.pos[t];
-  lo = window > 0 ? max(0, pos - window + 1) : 0;
-  hi = min(min(pos, 0x7FFFFFFE) + 1, P + pg.max_own);
+  pos = UNIFORM ? uload(pg.pos, t) : pg.pos[t];
+  lo = window > 0 ? max(0, max(pos, 0) - window + 1) : 0;
   return s >= 0 && s < pg.nseq && pos >= 0;
 }
 
@@ -512,10 +513,10 @@ struct PgRows {
     for (int r = 0; r < NR; ++r) {
       const int R = r0 + 16 * r + c, t = min(R, nrows - 1) / a.grp;
       load_q(a.q + (long)t * a.ldq + (long)(kvh * a.grp + min(R, nrows - 1) % a.grp) * HD + e0, g, qf[r]);
-      int s, lo, hi;
-      const bool live = pg_token<false>(pg, t, a.window, P, s, lo, hi) && R < nrows;
-      hi = min(hi, P);
-      pos[r] = live ? min(pg.pos[t], 0x7FFFFFFE) : -1;
+      int s, p, lo;
+      const bool live = pg_token<false>(pg, t, a.window, s, p, lo) && R < nrows;
+      const int hi = min(p, P - 1) + 1;
+      pos[r] = live ? p : -1;
       if (live) {
         if (lo < hi) blo = min(blo, lo), bhi = max(bhi, hi);
         wlo = max(wlo, lo), whi = min(whi, hi);
@@ -552,7 +553,7 @@ __device__ __forceinline__ void shared_role(const PgArgs& a, const Pages& pg, ui
   const int kvh = bid % a.nkv, split = bid / a.nkv % a.nsp, rb = bid / (a.nkv * a.nsp);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15,
             g = lane >> 4, dp = wave % DS;
-  const int P = pg.prefix(), r0 = (rb * PG_WAVES + wave / DS) * 16 * NR;
+  const int P = pg.prefix_keys(), r0 = (rb * PG_WAVES + wave / DS) * 16 * NR;
   v8h qf[NR][NCH];
   const PgRows<HD, NR, NCH> rows(a, pg, kvh, r0, dp * HW, P, qf);
   // the keys of all waves' rows: the whole prefix, which is known before the rows are, or the windows' part of it
@@ -689,20 +690,20 @@ __device__ __forceinline__ void stream_role(const PgArgs& a, const Pages& pg, ui
   const int nsplit = OWN ? a.nso : a.nsp, nhb = OWN ? a.nhb : 1;
   const int kvh = OWN ? item / (nsplit * nhb) % a.nkv : item % a.nkv, split = OWN ? item % nsplit : item / a.nkv;
   const int hb = OWN ? item / nsplit % nhb : 0, t = OWN ? item / (nsplit * nhb * a.nkv) : 0;
-  const int P = pg.prefix();
+  const int P = OWN ? pg.prefix() : pg.prefix_keys();
 
   // ---- rows, and the keys lo .. hi - 1 of them all (OWN: of the own pages) ----
   v8h qf[1][NCH];
-  int lo, hi, wlo, whi, pos = 0, heads = 16;  // pos: of the lane's prefix row
+  int lo, hi, wlo, whi, pos, heads = 16;  // pos: of the token, or of the lane's prefix row
   const int32_t* tab = pg.prefix_pages;
   if constexpr (OWN) {
     heads = min(a.grp - 16 * hb, 16);
     const int hc = HL ? c & 7 : c;
     load_q(a.q + (long)t * a.ldq + (long)(kvh * a.grp + 16 * hb + (hc < heads ? hc : 0)) * HD, g, qf[0]);
     int s;
-    if (!pg_token<true>(pg, t, a.window, P, s, lo, hi)) return;  // (uniform) no row
+    if (!pg_token<true>(pg, t, a.window, s, pos, lo)) return;  // (uniform) no row
     lo = max(0, lo - P);
-    hi -= P;
+    hi = min(pos - P, pg.max_own - 1) + 1;
     if (hi <= lo) lo = hi = 0;  // no keys (a position far past max_own: lo + split * per would pass 32 bits)
     tab = pg.table + (long)s * pg.ld;
     wlo = lo, whi = hi;
@@ -1000,7 +1001,7 @@ int q4_paged_prep(const void* qkv, int dtype, int ld, int qoff, int koff, int vo
   Q4_ARG(!overlap(kc, cache, vc, cache), "kc and vc must not overlap");
   for (const void* c : {kc, vc})
     Q4_ARG(!overlap(c, cache, q, nq) && !overlap(c, cache, qkv, nx), "the cache must not overlap q or qkv");
-  const Pages pg{nullptr, prefix_len, table, seq, pos, table_ld, nseq, npages, lg, 0x7FFFFFFF, 0};
+  const Pages pg{nullptr, prefix_len, table, seq, pos, table_ld, nseq, npages, lg, 0, 0};
   const int groups = 256 / (hd / 8), heads = nH + 2 * nkv;
   hipStream_t st = as_stream(stream);
   // heads per group of lanes: few where the workgroups do not fill the chip (64 rows of 16 + 2 x 8 heads of 256: 4.8 us

@@ -1125,9 +1125,11 @@ def paged_attn(q, kc, vc, out=None, *, nH: int, table, seq, pos, window: int = 0
     (int32), which every sequence shares and which are read once for all,
     the others in the sequence's own pages ``table[s]``. Returns ``out``
     [T][nH * hd] fp16 (rows of padding are left as they were; a row without
-    keys gives zeros, a query head with an Inf or NaN NaN). ``max_prefix`` and ``max_own`` bound the prefix and a
-    sequence's own keys for the launch plan (default: what the page arrays
-    hold); a graph may replay with other lengths below them. ``ws``:
+    keys gives zeros, a query head with an Inf or NaN NaN). ``max_prefix`` and
+    ``max_own`` bound the prefix and a sequence's own keys for the launch plan
+    (default: what the page arrays hold; keys past them are left out, and with
+    ``max_prefix`` 0 there is no prefix, whatever ``prefix_len`` holds); a
+    graph may replay with other lengths below them. ``ws``:
     :func:`paged_attn_workspace` of the same sizes (allocated here when
     omitted; capture code must pass its own where it is needed). Cache rows
     must be finite from the first to the last key attended there (own pages:

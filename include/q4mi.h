@@ -589,11 +589,12 @@ int q4_paged_prep(const void* qkv, int dtype, int ld, int qoff, int koff, int vo
  * 0), out[t][h hd ..] = softmax(q . K) V in fp16, no score scaling. The
  * prefix is read once for all rows. max_prefix and max_own bound P and a
  * sequence's own keys for the launch plan and the workspace (prefix_pages
- * holds ceil(max_prefix / page) entries; max_own <= table_ld * page; keys past
- * max_own are left out); max_prefix 0: no prefix, prefix_pages and prefix_len
- * unused. Keys without a page are left out; a row left without keys gives
- * zeros. A query head that holds an Inf or NaN gives NaN throughout, other
- * heads and rows their own outputs. Cache rows must be finite from the first to the last key attended
+ * holds ceil(max_prefix / page) entries; max_own <= table_ld * page; keys of
+ * the prefix past max_prefix and own keys past max_own are left out);
+ * max_prefix 0: no prefix, prefix_pages and prefix_len unused. Keys without a
+ * page are left out; a row left without keys gives zeros. A query head that
+ * holds an Inf or NaN gives NaN throughout, other heads and rows their own
+ * outputs. Cache rows must be finite from the first to the last key attended
  * there, by its row in own pages, by any row in the prefix (without a
  * window: the whole prefix); all others may hold anything. Softmax
  * statistics and sums in fp32; a weight enters the V product as the sum of two

@@ -12,10 +12,9 @@ subnormals).
 """
 import numpy as np
 import pytest
-import torch
 
 from oracle import paged_oracle as G
-from test_gpu_paged import F16, _attn_case, _np, _run_attn
+from test_gpu_paged import _attn_case, _i, _np, _run_attn
 
 pytestmark = pytest.mark.gpu
 
@@ -114,3 +113,53 @@ def test_nonfinite_queries_without_keys_give_zeros(gpu):
     c["pre"][:] = -1
     c["q"][1, 3], c["q"][1, 300] = np.nan, np.inf
     assert not _np(_run_attn(gpu, c))[1].any()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("form", [f for f in FORMS if FORMS[f][2]])
+@pytest.mark.parametrize("window", [0, 120])
+def test_prefix_longer_than_its_bound(gpu, form, hd, window):
+    """prefix_len divides the positions for the append and for attention
+    alike: past max_prefix its keys are left out, and own keys stay where
+    they are."""
+    c = _case(form, hd, 80, poison=False)
+    c["window"] = window
+    bound = 150     # of 300 positions: the fifth page in part
+    got = _np(_run_attn(gpu, dict(c, pre=c["pre"][:5]), max_prefix=bound)).astype(np.float64)
+    nkv, page = c["kc"].shape[1:3]
+    grp = c["nH"] // nkv
+    for t in range(len(c["q"])):
+        p = c["pos"][t]
+        keys = [j for j in range(max(0, p - window + 1) if window else 0, p + 1) if j < bound or j >= c["P"]]
+        pg, sl = np.array([G.slot(j, t, c["P"], c["table"], c["pre"], page, len(c["kc"])) for j in keys]).T
+        for h in range(c["nH"]):
+            sc = c["kc"][pg, h // grp, sl].astype(np.float64) @ c["q"][t, h * hd:(h + 1) * hd].astype(np.float64)
+            e = np.exp(sc - sc.max())
+            r = (e @ c["vc"][pg, h // grp, sl].astype(np.float64)) / e.sum()
+            off = np.abs(got[t, h * hd:(h + 1) * hd] - r) - (np.abs(r) * 2.0 ** -11 + 2.0 ** -25 +
+                                                             4e-5 * np.abs(c["vc"]).max())
+            assert (off <= 0).all(), (t, h, off.max())
+
+
+def test_prefix_length_of_any_value(gpu):
+    """Lengths up to 2^31 - 1 with the default bound, the 128 positions that the
+    prefix's pages hold: rows inside the prefix keep the keys below it."""
+    c = _attn_case(90, 16, 8, 256, 32, 100, [1, 2, 3, 4], 0, 0, poison=False)
+    for n in (2 ** 31 - 1, 2 ** 31 - 200, -5):
+        for window in (0, 30):
+            c.update(window=window, pos=[5, 99, 130, 2 ** 31 - 1])
+            got = _np(_run_attn(gpu, c, prefix_len=_i([n]), max_own=32)).astype(np.float64)
+            P = max(n, 0)
+            for t, p in enumerate(c["pos"]):
+                # own keys from P on, of which there are 32
+                near = [j for j in range(0, 128) if j < P and j <= p and (not window or j > p - window)]
+                near += [j for j in range(P, P + 32) if j <= p and (not window or j > p - window)]
+                r = np.zeros(16 * 256)
+                if near:
+                    pg, sl = np.array([G.slot(j, t, P, c["table"], c["pre"], 32, len(c["kc"])) for j in near]).T
+                    for h in range(16):
+                        sc = c["kc"][pg, h // 2, sl].astype(np.float64) @ c["q"][t, h * 256:(h + 1) * 256].astype(np.float64)
+                        e = np.exp(sc - sc.max())
+                        r[h * 256:(h + 1) * 256] = (e @ c["vc"][pg, h // 2, sl].astype(np.float64)) / e.sum()
+                off = np.abs(got[t] - r) - (np.abs(r) * 2.0 ** -11 + 2.0 ** -25 + 4e-5 * np.abs(c["vc"]).max())
+                assert (off <= 0).all(), (n, window, t, off.max())
