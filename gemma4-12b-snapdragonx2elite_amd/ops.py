@@ -962,7 +962,8 @@ def _current(t) -> int:
     return dev
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream   # of a device index; 60 ns against 2.5 us for a Stream object
+# of a device index; 60 ns against 2.5 us for a Stream object (a CPU-only torch has none, and no device tensors either)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _i8_rows(dev: int, M: int, D: int, A, sa):
