@@ -39,8 +39,8 @@ FILE_FLAGS = {"gemv.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
               # the online softmax rescales the attention accumulators every key tile: in AGPRs each
               # rescale moved them out and back (~20% of the loop's instructions)
               "prefill_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-              # the accumulators of head dim 512 take all AGPRs, so that scores, which would need AGPRs too
-              # without this, spilled 397 registers
+              # the same: without it the streams of head dim 512 keep 144 values in AGPRs (with it 3 to 7; the
+              # shared tiles, whose rows two waves share, none either way)
               "paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 

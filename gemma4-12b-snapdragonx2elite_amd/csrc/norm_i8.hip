@@ -75,9 +75,11 @@ __device__ inline void ni_reduce(float& a, float& b, float* red) {
 }
 
 // One row per workgroup, every operand in registers (NC chunks of 8 values
-// per thread). The largest |y| is the largest |h' w2| times inv(h'), so it
-// is reduced with the sum of squares: one barrier per norm. All loads are
-// issued before the first reduction. Bound by memory for many rows (2048 rows
+// per thread) up to D 16384; past it 1024 threads leave 128 registers each,
+// and the form with the residual, 128 values and more, spills 49 to 98. The
+// largest |y| is the largest |h' w2| times inv(h'), so it is reduced with the
+// sum of squares: one barrier per norm. All loads are issued before the first
+// reduction. Bound by memory for many rows (2048 rows
 // of 3840 with fp16 x and the residual: 86.5 MB in 17 us, 5 TB/s, the rate of a
 // copy, where part of it is in the cache; 22.7 us on cold data), by the launch
 // and one round trip of loads for few (one row 3.2 us, 128 rows 4.2 us).
@@ -192,7 +194,10 @@ static void ni_rows(const void* x, const float* w, float* h, int D, int M, float
   //   D  3840: 512 x 1 3.5 / 4.6 / 24.8, 256 x 2 3.6 / 4.7 / 25.1, 128 x 4 4.3 / 5.5 / 28.4, 1024 x 1 4.0 / 5.1 / 28.0
   //   D  5120: 512 x 2 4.0 / 5.3 / 32.4, 256 x 4 4.2 / 5.5 / 32.2, 1024 x 1 4.4 / 5.7 / 34.3
   //   D 15360: 512 x 4 6.9 / 12.6 / 97.7, 1024 x 2 7.0 / 12.8 / 99.3
-  // and single-element accesses of the same rows: 14.2 at D 2000, 25.7 at 3840, 42.7 at 5120, 106 at 15360 (2048 rows)
+  // and single-element accesses of the same rows: 14.2 at D 2000, 25.7 at 3840, 42.7 at 5120, 106 at 15360 (2048 rows);
+  // past D 16384 (4 chunks of 1024 threads, the residual form spilling), fp16 x, us per call from Python: D 20000
+  // 13.6 / 21.5 / 254 (single-element accesses, D 20001: 493 at 2048 rows), D 32768 17.6 / 30.3 / 322 (765 at 32767);
+  // without the residual D 32768 87.5 at 2048 rows
   if (D <= 2048) ni_launch<256, 1, ADD, XT>(x, w, h, D, M, sc, w2, A, sa, vec, st);
   else if (D <= 4096) ni_launch<512, 1, ADD, XT>(x, w, h, D, M, sc, w2, A, sa, vec, st);
   else if (D <= 8192) ni_launch<512, 2, ADD, XT>(x, w, h, D, M, sc, w2, A, sa, vec, st);

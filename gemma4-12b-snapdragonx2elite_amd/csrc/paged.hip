@@ -69,8 +69,8 @@ __device__ inline float pg_head_sum(float v) {
 // LPH = HD / 8 lanes: heads 0 .. nH - 1 are q, then nkv of k, then nkv of v.
 // A lane holds 8 elements, one 16-byte load of fp16 and one store; the RoPE
 // partner is the same slot of lane ^ LPH / 2. Bound by memory for large
-// batches (2048 rows of 16 + 2 heads of 512: 82 MB in 16.8 us, 4.9 TB/s, the
-// rate of a copy), else by the chain seq, pos -> RoPE row and page -> store
+// batches (2048 rows of 16 + 2 heads of 512: 82 MB in 15.6 to 17.1 us, 4.8 to
+// 5.3 TB/s, about the rate of a copy), else by the chain seq, pos -> RoPE row and page -> store
 // (one row of 16 + 2 x 8 heads of 256 among others: 3.8 us).
 template <int HD, int DT, int HPG>
 __global__ void __launch_bounds__(256)
@@ -147,13 +147,13 @@ constexpr int PG_THREADS = 256, PG_WAVES = 4;
 // stream.
 enum { PG_OWN, PG_SHARED, PG_SHARED_FEW, PG_STREAM };
 // Most rows of a prefix that streams: 16, a wave's MFMA columns. us with the merge behind 16384 (4096) keys, as streams
-// and in shared tiles: 8 heads of 256, 2 rows 29.5 / 32.0 and 16 rows 31.7 / 34.2 (15.9 / 16.5); one of 512, 16 rows
-// 23.2 / 23.8 (15.3 / 14.6); 8 of 128, 4 rows 19.8 / 20.6 (9.0 / 9.3).
+// and in shared tiles, each launch alone: 8 heads of 256, 2 rows 33.0 / 35.5 (17.5 / 17.6) and 16 rows 35.4 / 38.1
+// (17.4 / 18.0); one of 512, 16 rows 24.0 / 23.4 (16.4 / 15.6); 8 of 128, 16 rows 20.4 / 21.1 (12.4 / 12.3).
 constexpr int PG_STREAM_ROWS = 16;
 // Most rows of a workgroup of 16 rows per wave, which leaves waves busy where 32 would leave them without rows; with
-// more rows than it holds each tile would be loaded again. us behind 16384 keys with 16 and with 32 rows per wave: 8
-// heads of 256, 32 rows 36.1 / 37.3 and 64 rows 39.0 / 41.5; one of 512, 24.2 / 28.1 and 27.7 / 32.5; 8 of 128, 22.4 /
-// 23.4 and 24.1 / 27.1.
+// more rows than it holds each tile would be loaded again. us with the merge behind 16384 keys with 16 and with 32 rows
+// per wave: 8 heads of 256, 32 rows 42.7 / 43.6 and 64 rows 51.4 / 52.4; one of 512, 24.2 / 28.5 and 28.2 / 33.9; 8 of
+// 128, 22.7 / 24.0 and 26.2 / 29.2.
 constexpr int PG_FEW_ROWS = 64;
 constexpr float PG_LOG2E = 1.4426950408889634f;
 // A row's weights are 2^(score - ref): ref is set 6 below the row's largest
@@ -533,16 +533,21 @@ struct PgRows {
 // NR groups of 16 rows per wave. Up to head dim 256 a wave holds its rows by
 // itself; behind a long prefix the cache's bytes bound it (8 rows of 32 heads
 // of 128 behind 32001 keys and 150 own: 134 MB in 32 us, 4.2 TB/s; its loads
-// and barriers alone 24.3, and a start of ~3 us before the first tile). Head
-// dim 512 takes two waves per NR groups, each with half of the elements: of q for the scores, whose
-// halves the pair adds through LDS, and of the outputs. So a wave's registers
-// stay within 256 and two waves share a SIMD (one wave of 465 registers
-// issued at most one instruction per 4 cycles, 840 a tile beside 2k cycles of
-// MFMAs: 76 us per 23.8k keys for 64 rows of 16 heads, with pairs 68). What
-// bounds it then (64 rows of 16 heads behind 8192 keys and up to 1000 own: 58
-// us, 18.2 GFLOP): softmax, score exchange and barriers beside the matrix
-// products, with one workgroup's 160 KB of LDS per CU nothing to run under
-// them (tile loads alone take 22.6 of 40 us, all but the loads 33).
+// and barriers alone 24.3, and a start of ~3 us before the first tile); with
+// many rows the weights' second parts show (64 rows there: 72 us, with weights
+// of one fp16 value 61). Head dim 512 takes two waves per NR groups, each with
+// half of the elements: of q for the scores, whose halves the pair adds
+// through LDS, and of the outputs. So a wave's registers stay within 256 and
+// two waves share a SIMD (one wave of 465 registers issued at most one
+// instruction per 4 cycles, 840 a tile beside 2k cycles of MFMAs: with weights
+// of one fp16 value 76 us per 23.8k keys for 64 rows of 16 heads, with pairs
+// 68). What bounds it then (64 rows of 16 heads behind 32000 keys: 135 us, 3.3
+// per 1000 keys; with weights of one value 113 and 2.7): softmax, score
+// exchange and barriers beside the matrix products, with one workgroup's 160
+// KB of LDS per CU nothing to run under them. Behind 8192 keys and up to 1000
+// own (60 us, 18.2 GFLOP) it is the grid: the plan's 160 workgroups of the
+// prefix take 58 us by themselves, on 160 of 256 CUs, where 8192 keys over all
+// CUs would take 27; the own pages alone take 18.5.
 template <int HD, int NR>
 __device__ __forceinline__ void shared_role(const PgArgs& a, const Pages& pg, uint32_t lds, uint32_t xs, int bid) {
   using S = PgTile<HD>;
@@ -854,7 +859,7 @@ paged_attn_kernel(const PgArgs a, const Pages pg) {
 // the row's parts, e_i = 2^(ref_i - largest ref), parts without keys left out.
 // Groups of lanes take every NG-th part, 4 elements (8 at HD 512) per lane.
 // Bound by the launch and one round trip of loads for few parts (3.5 - 5 us),
-// by the parts' bytes for many (1024 rows of 512 in 7 parts or more: 10.4 us).
+// by the parts' bytes for many (1024 rows of 512 in 24 parts: 10.4 us).
 constexpr int PG_MAX_PARTS = 512;
 template <int HD>
 __global__ void __launch_bounds__(PG_THREADS) paged_merge_kernel(const PgArgs a, const Pages pg) {
@@ -926,9 +931,9 @@ __global__ void __launch_bounds__(PG_THREADS) paged_merge_kernel(const PgArgs a,
 //  * prefix: more splits fill the chip, but each takes a part through memory,
 //    8 hd bytes per row out and in. With a time per key and one per part the
 //    sum is least at a square root of the keys per row; its factor is measured
-//    (64 rows of 16 heads of 512 behind 8192 keys, with the merge: 25 74.5 us,
-//    50 69.0, 100 74.7; 18 rows of 16 heads of 256 behind 2000: 19.3, 18.3,
-//    18.2; 8 rows of 32 heads of 128 behind 32001: 39.5, 38.9, 39.4); at least
+//    (64 rows of 16 heads of 512 behind 8192 keys, with the merge: 25 85.0 us,
+//    50 70.9, 100 80.6; 18 rows of 16 heads of 256 behind 2000: 17.0, 16.9,
+//    16.5; 8 rows of 32 heads of 128 behind 32001: 37.8, 37.1, 37.3); at least
 //    two tiles per split.
 //  * own: up to 4 rounds of workgroups while a split keeps 8 tiles per wave, so
 //    that ragged lengths even out.

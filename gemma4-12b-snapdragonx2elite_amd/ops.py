@@ -1066,7 +1066,8 @@ def paged_prep(qkv, qnw, knw, cos_tab, sin_tab, kc, vc, q=None, *, nH: int, koff
     ``qkv`` [T][...] (fp32 or fp16; q, k, v at element offsets ``qoff``,
     ``koff``, ``voff`` of a row, ``voff == koff`` where v is k). Row t is
     position ``pos[t]`` of sequence ``seq[t]`` (int32; a negative ``seq`` or
-    a position past the RoPE tables marks padding, left alone). Returns ``q``
+    a position past the RoPE tables marks padding, left alone; for
+    :func:`paged_attn` only the former does). Returns ``q``
     [T][nH * hd] fp16, normed with ``qnw`` and rotated; k (normed with
     ``knw``, rotated) and v (normed) are appended to the cache ``kc``, ``vc``
     [pages][nkv][page][hd] at the sequence's own pages ``table``

@@ -555,7 +555,7 @@ int q4_pre_normadd_rmsnorm_i8(const void* x, int x_dtype, const float* w, float*
 /* ---- batched decode on a paged KV cache ---------------------------------------
  * T rows, one token each: row t is position pos[t] of sequence seq[t]; a
  * row whose seq is outside 0 .. nseq-1 or whose pos is negative is no row
- * (padding): nothing of it is read or written. Caches kc, vc: fp16
+ * (padding): nothing of it is used or written. Caches kc, vc: fp16
  * [npages][nkv][page][hd], page a power of two of 16 .. 4096. With
  * P = prefix_len[0] (0 for a NULL prefix_len), position j < P is row
  * j % page of page prefix_pages[j / page], shared by all sequences; a later
@@ -571,7 +571,8 @@ int q4_pre_normadd_rmsnorm_i8(const void* x, int x_dtype, const float* w, float*
  * [T][ldq]; K = f16 of RoPE(rmsnorm(k) * knw) and V = f16 of rmsnorm(v) into
  * the sequence's own page at pos (nothing where pos < P, past the table, or
  * no page). RoPE rows cos_tab, sin_tab [max_pos][hd] at pos; a row with
- * pos >= max_pos is no row. Two rows must not name one cache slot (either
+ * pos >= max_pos is no row here (attention does not know max_pos: it needs a
+ * seq of -1 there too, or takes whatever q holds). Two rows must not name one cache slot (either
  * one's 16-byte pieces may end there). All pointers but the int32 arrays
  * 16-byte aligned; ld and the offsets multiples of 16 bytes, ldq a multiple
  * of 8; q, qkv, kc and vc may not overlap, each taken from its first to its
